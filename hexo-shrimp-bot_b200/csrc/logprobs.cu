@@ -542,8 +542,13 @@ extern "C" int mb_log_probs_backward(const void* logits, int dtype, int64_t n, c
   MB_REQUIRE(n >= 0 && n_segments >= 0, "log_probs_backward: negative size");
   MB_REQUIRE(top >= 0 && top <= logp::kMaxTop, "log_probs_backward: top must be in [0, %d] (got %d)", logp::kMaxTop,
              top);
-  if (n_segments == 0 || n == 0) return MB_OK;
-  MB_REQUIRE(logits && offsets && lse && entropy && grad && (top == 0 || (top_ranks && g_top)),
+  if (n == 0) return MB_OK;
+  MB_REQUIRE(grad, "log_probs_backward: null pointer");
+  if (n_segments == 0) {  // every element is outside every segment
+    (void)cudaMemsetAsync(grad, 0, (size_t)n * dtype_size(dtype), as_stream(stream));
+    return launch_status("log_probs_backward");
+  }
+  MB_REQUIRE(logits && offsets && lse && entropy && (top == 0 || (top_ranks && g_top)),
              "log_probs_backward: null pointer");
   MB_REQUIRE(aligned(logits, dtype_size(dtype)) && ((uintptr_t)logits & 15) == ((uintptr_t)grad & 15),
              "log_probs_backward: logits and grad must be aligned alike");
