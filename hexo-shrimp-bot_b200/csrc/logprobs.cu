@@ -259,6 +259,11 @@ __device__ __noinline__ void warp_lists(Lists& ls, const T* base, int64_t vb, in
   __syncthreads();
 }
 
+// Ranks have 32 bits.
+__device__ __forceinline__ bool malformed(int64_t a, int64_t b, int64_t n) {
+  return a < 0 || b < a || b > n || b - a > 0xffffffffLL;
+}
+
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kMaxThreads, TOP ? 4 : 6) forward_kernel(
     const T* __restrict__ logits, int64_t n, const int64_t* __restrict__ offsets, const int64_t* __restrict__ ranks,
@@ -273,7 +278,7 @@ __global__ void __launch_bounds__(kMaxThreads, TOP ? 4 : 6) forward_kernel(
   const int64_t p = blockIdx.x / split;
   const int part = blockIdx.x % split;
   int64_t a = offsets[p], b = offsets[p + 1];
-  if (a < 0 || b < a || b > n || b - a > 0xffffffffLL) {
+  if (malformed(a, b, n)) {
     if (tid == 0) report(ERR_RUN_BOUND);
     a = b = 0;
   }
@@ -393,6 +398,45 @@ __global__ void __launch_bounds__(kMaxThreads, TOP ? 4 : 6) forward_kernel(
   }
 }
 
+// A malformed segment reads as empty, in both directions. Its offsets may leave
+// elements to no segment at all, whose gradient is zero: this one clears, of
+// those between the highest offset so far and its own end, the ones that no well-
+// formed segment holds. Offsets that pass an element for the first time do so
+// in such a step or in a well-formed segment, so all are written; the first and
+// last segment clear what lies outside all offsets. Off the ordinary path: every
+// step here reads the offsets, and no element is cleared twice.
+template <typename T>
+__device__ __noinline__ void zero_malformed(const int64_t* __restrict__ offsets, int64_t n_segments, int64_t p,
+                                            int64_t n, T* __restrict__ grad) {
+  __shared__ long long reach, next;
+  const long long end = min(max(offsets[p + 1], (int64_t)0), n);
+  if (threadIdx.x == 0) reach = 0;
+  __syncthreads();
+  for (int64_t i0 = p; i0 >= 0; i0 -= blockDim.x) {  // the highest offset so far
+    const int64_t i = i0 - threadIdx.x;
+    const long long o = i >= 0 ? min(max(offsets[i], (int64_t)0), n) : 0;
+    atomicMax(&reach, o);
+    if (__syncthreads_or(o >= end)) return;
+  }
+  long long at = reach;
+  while (at < end) {
+    __syncthreads();
+    if (threadIdx.x == 0) reach = at, next = end;
+    __syncthreads();
+    for (int64_t i = threadIdx.x; i < n_segments; i += blockDim.x) {
+      const long long a = offsets[i], b = offsets[i + 1];
+      if (malformed(a, b, n) || b <= at) continue;
+      if (a <= at) atomicMax(&reach, b);
+      else atomicMin(&next, a);
+    }
+    __syncthreads();
+    const long long held = reach, to = next;
+    if (held == at)
+      for (long long e = at + threadIdx.x; e < to; e += blockDim.x) grad[e] = from_f<T>(0.f);
+    at = held > at ? held : to;
+  }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kMaxThreads, 8) backward_kernel(
     const T* __restrict__ logits, int64_t n, const int64_t* __restrict__ offsets, const int64_t* __restrict__ ranks,
@@ -406,16 +450,17 @@ __global__ void __launch_bounds__(kMaxThreads, 8) backward_kernel(
   const int64_t p = blockIdx.x / split;
   const int part = blockIdx.x % split;
   const int64_t a = offsets[p], b = offsets[p + 1];
-  if (a < 0 || b < a || b > n) {
-    if (tid == 0) report(ERR_RUN_BOUND);
-    return;
-  }
   // elements outside every segment have no gradient
   if (part == 0) {
     if (p == 0)
-      for (int64_t e = tid; e < a; e += blockDim.x) grad[e] = from_f<T>(0.f);
+      for (int64_t e = tid; e < min(a, n); e += blockDim.x) grad[e] = from_f<T>(0.f);
     if ((p + 1) * split == gridDim.x)
-      for (int64_t e = b + tid; e < n; e += blockDim.x) grad[e] = from_f<T>(0.f);
+      for (int64_t e = max(b, (int64_t)0) + tid; e < n; e += blockDim.x) grad[e] = from_f<T>(0.f);
+  }
+  if (malformed(a, b, n)) {
+    if (tid == 0) report(ERR_RUN_BOUND);
+    if (part == 0) zero_malformed(offsets, gridDim.x / split, p, n, grad);
+    return;
   }
   if (b == a) return;
   // the elements with a gradient of their own: the chosen one, then the listed ones

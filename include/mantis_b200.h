@@ -544,8 +544,8 @@ int mb_log_probs(const void* logits, int dtype, int64_t n, const int64_t* offset
                  float* top_logp, void* stream);
 
 /* Gradient of sum_s (g_logp logp + g_entropy entropy + sum_k g_top top_logp)
- * over the logits, in their type (zero outside every segment; grad aligned
- * modulo 16 as logits). g_logp and g_entropy (n_segments) may be NULL
+ * over the logits, in their type (zero outside every segment and in a
+ * malformed one; grad aligned modulo 16 as logits). g_logp and g_entropy (n_segments) may be NULL
  * (zero); top and top_ranks from the forward call with g_top, or top 0. */
 int mb_log_probs_backward(const void* logits, int dtype, int64_t n, const int64_t* offsets, int64_t n_segments,
                           const int64_t* ranks, int top, const float* lse, const float* entropy,

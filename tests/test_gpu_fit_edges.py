@@ -32,3 +32,34 @@ def test_log_probs_gradient_without_segments(dtype, n):
     _stale(n + 8, x.dtype)
     dx = ops.log_probs_backward(x, off, None, got, torch.zeros(0, device=DEV))
     assert dx.shape == x.shape and torch.count_nonzero(dx) == 0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,offsets,well", [
+    (133, (0, 200, 133), ()), (133, (-5, 40, 133), (1,)), (133, (0, 50, 140), (0,)), (133, (0, 50, -3, 133), (0,)),
+    (133, (150, 133, 133), ()), (70001, (0, 70002), ()), (70001, (0, 70002, 65000, 70001), (2,))])
+def test_log_probs_gradient_of_malformed_segments(dtype, n, offsets, well):
+    """A malformed segment is an error, and its elements have no gradient; the
+    others' are what they are without it."""
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn(n, generator=g).to(DT[dtype]).to(DEV)
+    off = torch.tensor(offsets, device=DEV)
+    p = off.shape[0] - 1
+    gl, ge, gt = (torch.randn(*s, generator=g).to(DEV) for s in ((p,), (p,), (p, 3)))
+    got = ops.log_probs(x, off, torch.zeros(p, dtype=torch.int64, device=DEV) - 1, top=3)
+    with pytest.raises(ValueError, match="malformed"):
+        mb._lib.check_device_error()
+    _stale(n + 8, x.dtype)
+    dx = ops.log_probs_backward(x, off, None, got, gl, ge, gt)
+    with pytest.raises(ValueError, match="malformed"):
+        mb._lib.check_device_error()
+    want = torch.zeros_like(dx)
+    for s in well:
+        a, b = offsets[s], offsets[s + 1]
+        one = torch.tensor([0, b - a], device=DEV)
+        part = x[a:b].clone()
+        alone = ops.log_probs(part, one, None, top=3)
+        want[a:b] = ops.log_probs_backward(part, one, None, alone, gl[s:s + 1], ge[s:s + 1], gt[s:s + 1].contiguous())
+    # the statistics' sums may be split otherwise: 2^-20 of terms of a few units, and a step of the type
+    torch.testing.assert_close(dx.float(), want.float(), rtol=2.0 ** -7 if dtype == "bf16" else 2.0 ** -18, atol=2.0 ** -18)
+    mb._lib.check_device_error()
