@@ -368,7 +368,7 @@ def _save_bucket_attention(ctx, inputs, output):
 
 def _bw_bucket_attention(ctx, g_out, g_lse, g_full):
     q, k, v, bias, bucket_map, coords, valid, out, lse, full = ctx.saved_tensors
-    stats = ops.AttentionStats(lse, full if full.numel() or not out.numel() else None)
+    stats = ops.AttentionStats(lse, full if q.dtype == torch.bfloat16 else None)
     dq, dk, dv, dbias = ops.bucket_attention_backward(q, k, v, bias, bucket_map, coords, valid, out, stats, g_out,
                                                       scale=ctx.scale, bias_grad=ctx.needs_input_grad[3])
     return dq, dk, dv, dbias, None, None, None, None

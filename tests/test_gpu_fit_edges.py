@@ -3,6 +3,8 @@ forms and paths that ordinary sizes do not reach, and their torch ops."""
 
 from __future__ import annotations
 
+import importlib
+
 import pytest
 import torch
 
@@ -63,3 +65,29 @@ def test_log_probs_gradient_of_malformed_segments(dtype, n, offsets, well):
     # the statistics' sums may be split otherwise: 2^-20 of terms of a few units, and a step of the type
     torch.testing.assert_close(dx.float(), want.float(), rtol=2.0 ** -7 if dtype == "bf16" else 2.0 ** -18, atol=2.0 ** -18)
     mb._lib.check_device_error()
+
+
+# ------------------------------------------------------- the ops' autograd
+torch_ops = importlib.import_module("hexo-shrimp-bot_b200.torch_ops")
+torch_ops.define_fit()
+fit = torch.ops.mantis_b200
+
+
+def _attention_inputs(p, h, kv, length, d, dtype, seed=0, valid=None):
+    """q, k, v (with gradients), bias, bucket map, coordinates, valid."""
+    g = torch.Generator().manual_seed(seed)
+    q, k, v = (torch.randn(p, n, length, d, generator=g).to(DT[dtype]).to(DEV).requires_grad_() for n in (h, kv, kv))
+    bmap = torch.from_numpy(mb.hexgraph.displacement_buckets()).to(DEV)
+    bias = torch.randn(int(bmap.max()) + 1, h, generator=g).to(DEV).requires_grad_()
+    coords = torch.randint(-9, 10, (p, length, 2), generator=g, dtype=torch.int32).to(DEV)
+    return q, k, v, bias, bmap, coords, valid
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("p,length", [(0, 5), (2, 0), (0, 0)])
+def test_attention_autograd_of_an_empty_batch(dtype, p, length):
+    args = _attention_inputs(p, 4, 2, length, 32, dtype)
+    out = fit.bucket_attention(*args)[0]
+    grads = torch.autograd.grad(out.float().sum(), args[:4])
+    for x, y in zip(grads, args):
+        assert x.shape == y.shape and x.dtype == y.dtype and torch.count_nonzero(x) == 0
