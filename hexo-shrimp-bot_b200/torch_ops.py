@@ -363,10 +363,14 @@ _FIT_FAKES = {"bucket_attention": _fake_bucket_attention, "dropout_add": _fake_d
 
 def _save_bucket_attention(ctx, inputs, output):
     q, k, v, bias, bucket_map, coords, valid, ctx.scale = inputs
+    ctx.mark_non_differentiable(*output[1:])
+    ctx.set_materialize_grads(False)  # the aux outputs' zeros would be as large as out's
     ctx.save_for_backward(q, k, v, bias, bucket_map, coords, valid, *output)
 
 
 def _bw_bucket_attention(ctx, g_out, g_lse, g_full):
+    if g_out is None:
+        return (None,) * 8
     q, k, v, bias, bucket_map, coords, valid, out, lse, full = ctx.saved_tensors
     stats = ops.AttentionStats(lse, full if q.dtype == torch.bfloat16 else None)
     dq, dk, dv, dbias = ops.bucket_attention_backward(q, k, v, bias, bucket_map, coords, valid, out, stats, g_out,
@@ -384,6 +388,8 @@ def _bw_dropout_add(ctx, g):
 
 
 def _save_log_probs(ctx, inputs, output):
+    ctx.mark_non_differentiable(*output[2:4])
+    ctx.set_materialize_grads(False)
     ctx.save_for_backward(*inputs[:3], *output)
 
 
@@ -404,8 +410,8 @@ def define_fit(namespace: str = "mantis_b200") -> list[str]:
     """Define the fit operators in ``namespace`` with this library's CUDA
     kernels, fakes and autograd. ``bucket_attention`` returns (out, lse, full):
     the log-sum-exp and the unrounded output are kept for the backward pass
-    and carry no gradient; so does ``log_probs``'s lse (its logp, entropy and
-    top_logp do). Returns the qualified op names. Idempotent."""
+    and are not differentiable (``requires_grad`` is False), nor is
+    ``log_probs``'s lse (its logp, entropy and top_logp are). Returns the qualified op names. Idempotent."""
     names = [f"{namespace}::{n}" for n in _FIT_SCHEMAS]
     key = f"{namespace} (fit)"
     if key in _libs:

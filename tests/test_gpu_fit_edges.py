@@ -91,3 +91,38 @@ def test_attention_autograd_of_an_empty_batch(dtype, p, length):
     grads = torch.autograd.grad(out.float().sum(), args[:4])
     for x, y in zip(grads, args):
         assert x.shape == y.shape and x.dtype == y.dtype and torch.count_nonzero(x) == 0
+
+
+def _segment_inputs(dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(50, generator=g).to(DT[dtype]).to(DEV).requires_grad_()
+    return x, torch.tensor([0, 20, 50], device=DEV), torch.tensor([3, 29], device=DEV), 2
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_outputs_without_a_gradient_formula(dtype):
+    """A loss on a log-sum-exp raises; outputs that a loss leaves out cost the
+    backward pass no zeros (the unrounded output's would be 4 MiB here)."""
+    args = _attention_inputs(2, 4, 2, 4096, 32, dtype)
+    out, lse, full = fit.bucket_attention(*args)
+    seg = _segment_inputs(dtype)
+    logp, entropy, seg_lse, top, top_logp = fit.log_probs(*seg)
+    for aux in (lse, full, seg_lse):
+        assert not aux.requires_grad
+        with pytest.raises(RuntimeError, match="does not require grad"):
+            aux.sum().backward()
+    (dx,) = torch.autograd.grad(entropy.sum(), seg[0], retain_graph=True)
+    want = ops.log_probs_backward(seg[0].detach(), *seg[1:3], ops.log_probs(*seg[:3], top=2), None,
+                                  torch.ones(2, device=DEV))
+    assert torch.equal(dx, want)
+    go = torch.randn_like(out)
+    stats = ops.AttentionStats(lse, full if dtype == "bf16" else None)
+    peaks = []
+    for run in (lambda: ops.bucket_attention_backward(*args, out.detach(), stats, go),
+                lambda: torch.autograd.grad(out, args[:4], go)):
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        with torch.no_grad():
+            run()
+        peaks.append(torch.cuda.max_memory_allocated() - before)
+    assert peaks[1] <= peaks[0] + (1 << 20)
