@@ -31,6 +31,8 @@ probabilities of chosen moves), with fakes and autograd.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 from torch import Tensor
 
@@ -318,12 +320,23 @@ _AUTOGRAD = {
 
 
 # ------------------------------------------------------------ fit operators
+# Each differentiable op, and the op that its backward formula calls: an op of
+# its own, so that a traced backward pass keeps it opaque too. Seeds and
+# offsets are symbolic: they change every step, and a compiled one stays.
 _FIT_SCHEMAS = {
     "bucket_attention": ("(Tensor q, Tensor k, Tensor v, Tensor bias, Tensor bucket_map, Tensor coords, "
                          "Tensor? valid, float? scale=None) -> (Tensor, Tensor, Tensor)"),
-    "dropout_add": "(Tensor x, Tensor y, float p, int seed, int offset) -> Tensor",
+    "dropout_add": "(Tensor x, Tensor y, float p, SymInt seed, SymInt offset) -> Tensor",
     "log_probs": ("(Tensor logits, Tensor offsets, Tensor ranks, int top=0) "
                   "-> (Tensor, Tensor, Tensor, Tensor, Tensor)"),
+}
+_FIT_BACKWARD_SCHEMAS = {
+    "bucket_attention_backward": ("(Tensor q, Tensor k, Tensor v, Tensor bias, Tensor bucket_map, Tensor coords, "
+                                  "Tensor? valid, Tensor out, Tensor lse, Tensor full, Tensor grad_out, "
+                                  "float? scale=None, bool bias_grad=True) -> (Tensor, Tensor, Tensor, Tensor)"),
+    "dropout_backward": "(Tensor grad, float p, SymInt seed, SymInt offset, ScalarType dtype) -> Tensor",
+    "log_probs_backward": ("(Tensor logits, Tensor offsets, Tensor ranks, Tensor lse, Tensor entropy, Tensor top, "
+                           "Tensor? g_logp, Tensor? g_entropy, Tensor? g_top_logp) -> Tensor"),
 }
 
 
@@ -333,12 +346,26 @@ def _fit_bucket_attention(q, k, v, bias, bucket_map, coords, valid, scale=None):
     return out, stats.lse, full
 
 
+def _fit_bucket_attention_backward(q, k, v, bias, bucket_map, coords, valid, out, lse, full, grad_out, scale=None,
+                                   bias_grad=True):
+    stats = ops.AttentionStats(lse, full if q.dtype == torch.bfloat16 else None)
+    dq, dk, dv, dbias = ops.bucket_attention_backward(q, k, v, bias, bucket_map, coords, valid, out, stats, grad_out,
+                                                      scale=scale, bias_grad=bias_grad)
+    return dq, dk, dv, bias.new_empty(0) if dbias is None else dbias
+
+
 def _fit_log_probs(logits, offsets, ranks, top=0):
     return tuple(ops.log_probs(logits, offsets, ranks, top=top))
 
 
+def _fit_log_probs_backward(logits, offsets, ranks, lse, entropy, top, g_logp, g_entropy, g_top_logp):
+    got = ops.LogProbs(lse, entropy, lse, top, top)  # of its values the kernel reads lse, entropy and top
+    return ops.log_probs_backward(logits, offsets, ranks, got, g_logp, g_entropy, g_top_logp)
+
+
 _FIT_KERNELS = {"bucket_attention": _fit_bucket_attention, "dropout_add": ops.dropout_add,
-                "log_probs": _fit_log_probs}
+                "log_probs": _fit_log_probs, "bucket_attention_backward": _fit_bucket_attention_backward,
+                "dropout_backward": ops.dropout_backward, "log_probs_backward": _fit_log_probs_backward}
 
 
 def _fake_bucket_attention(q, k, v, bias, bucket_map, coords, valid, scale=None):
@@ -347,8 +374,18 @@ def _fake_bucket_attention(q, k, v, bias, bucket_map, coords, valid, scale=None)
             q.new_empty(full, dtype=torch.float32))
 
 
+def _fake_bucket_attention_backward(q, k, v, bias, bucket_map, coords, valid, out, lse, full, grad_out, scale=None,
+                                    bias_grad=True):
+    return (q.new_empty(q.shape), k.new_empty(k.shape), k.new_empty(k.shape),
+            bias.new_empty(bias.shape if bias_grad else 0))
+
+
 def _fake_dropout_add(x, y, p, seed, offset):
     return x.new_empty(x.shape)
+
+
+def _fake_dropout_backward(grad, p, seed, offset, dtype):
+    return grad.new_empty(grad.shape, dtype=dtype)
 
 
 def _fake_log_probs(logits, offsets, ranks, top=0):
@@ -357,10 +394,16 @@ def _fake_log_probs(logits, offsets, ranks, top=0):
     return f(p), f(p), f(p), logits.new_empty((p, top), dtype=torch.long), f(p, top)
 
 
+def _fake_log_probs_backward(logits, offsets, ranks, lse, entropy, top, g_logp, g_entropy, g_top_logp):
+    return logits.new_empty(logits.shape)
+
+
 _FIT_FAKES = {"bucket_attention": _fake_bucket_attention, "dropout_add": _fake_dropout_add,
-              "log_probs": _fake_log_probs}
+              "log_probs": _fake_log_probs, "bucket_attention_backward": _fake_bucket_attention_backward,
+              "dropout_backward": _fake_dropout_backward, "log_probs_backward": _fake_log_probs_backward}
 
 
+# The backward formulas call the backward op of the forward op's namespace.
 def _save_bucket_attention(ctx, inputs, output):
     q, k, v, bias, bucket_map, coords, valid, ctx.scale = inputs
     ctx.mark_non_differentiable(*output[1:])
@@ -368,14 +411,11 @@ def _save_bucket_attention(ctx, inputs, output):
     ctx.save_for_backward(q, k, v, bias, bucket_map, coords, valid, *output)
 
 
-def _bw_bucket_attention(ctx, g_out, g_lse, g_full):
+def _bw_bucket_attention(op, ctx, g_out, g_lse, g_full):
     if g_out is None:
         return (None,) * 8
-    q, k, v, bias, bucket_map, coords, valid, out, lse, full = ctx.saved_tensors
-    stats = ops.AttentionStats(lse, full if q.dtype == torch.bfloat16 else None)
-    dq, dk, dv, dbias = ops.bucket_attention_backward(q, k, v, bias, bucket_map, coords, valid, out, stats, g_out,
-                                                      scale=ctx.scale, bias_grad=ctx.needs_input_grad[3])
-    return dq, dk, dv, dbias, None, None, None, None
+    dq, dk, dv, dbias = op(*ctx.saved_tensors, g_out, ctx.scale, ctx.needs_input_grad[3])
+    return dq, dk, dv, dbias if ctx.needs_input_grad[3] else None, None, None, None, None
 
 
 def _save_dropout_add(ctx, inputs, output):
@@ -383,46 +423,50 @@ def _save_dropout_add(ctx, inputs, output):
     ctx.y_dtype = y.dtype
 
 
-def _bw_dropout_add(ctx, g):
-    return g, ops.dropout_backward(g, ctx.p, ctx.seed, ctx.offset, dtype=ctx.y_dtype), None, None, None
+def _bw_dropout_add(op, ctx, g):
+    return g, op(g, ctx.p, ctx.seed, ctx.offset, ctx.y_dtype), None, None, None
 
 
 def _save_log_probs(ctx, inputs, output):
     ctx.mark_non_differentiable(*output[2:4])
     ctx.set_materialize_grads(False)
-    ctx.save_for_backward(*inputs[:3], *output)
+    ctx.save_for_backward(*inputs[:3], output[2], output[1], output[3])
 
 
-def _bw_log_probs(ctx, g_logp, g_entropy, g_lse, g_top, g_top_logp):
-    logits, offsets, ranks, *got = ctx.saved_tensors
+def _bw_log_probs(op, ctx, g_logp, g_entropy, g_lse, g_top, g_top_logp):
     grads = [None if g is None else g.float().contiguous() for g in (g_logp, g_entropy, g_top_logp)]
     if grads[2] is not None and grads[2].numel() == 0:
         grads[2] = None
-    return ops.log_probs_backward(logits, offsets, ranks, ops.LogProbs(*got), *grads), None, None, None
+    return op(*ctx.saved_tensors, *grads), None, None, None
 
 
 _FIT_AUTOGRAD = {"bucket_attention": (_bw_bucket_attention, _save_bucket_attention),
                  "dropout_add": (_bw_dropout_add, _save_dropout_add),
                  "log_probs": (_bw_log_probs, _save_log_probs)}
+_FIT_BACKWARD_OP = {"bucket_attention": "bucket_attention_backward", "dropout_add": "dropout_backward",
+                    "log_probs": "log_probs_backward"}
 
 
 def define_fit(namespace: str = "mantis_b200") -> list[str]:
     """Define the fit operators in ``namespace`` with this library's CUDA
-    kernels, fakes and autograd. ``bucket_attention`` returns (out, lse, full):
+    kernels, fakes and autograd; their backward passes are ops with fakes too, so
+    a training step traces. ``bucket_attention`` returns (out, lse, full):
     the log-sum-exp and the unrounded output are kept for the backward pass
     and are not differentiable (``requires_grad`` is False), nor is
-    ``log_probs``'s lse (its logp, entropy and top_logp are). Returns the qualified op names. Idempotent."""
+    ``log_probs``'s lse (its logp, entropy and top_logp are). Returns the
+    differentiable ops' qualified names. Idempotent."""
     names = [f"{namespace}::{n}" for n in _FIT_SCHEMAS]
     key = f"{namespace} (fit)"
     if key in _libs:
         return names
     lib = torch.library.Library(namespace, "FRAGMENT")
-    for name, schema in _FIT_SCHEMAS.items():
-        qual = f"{namespace}::{name}"
+    for name, schema in {**_FIT_SCHEMAS, **_FIT_BACKWARD_SCHEMAS}.items():
         lib.define(name + schema)
         lib.impl(name, _FIT_KERNELS[name], "CUDA")
-        torch.library.register_fake(qual, _FIT_FAKES[name], lib=lib)
-        backward, setup = _FIT_AUTOGRAD[name]
-        torch.library.register_autograd(qual, backward, setup_context=setup, lib=lib)
+        torch.library.register_fake(f"{namespace}::{name}", _FIT_FAKES[name], lib=lib)
+    for name, (backward, setup) in _FIT_AUTOGRAD.items():
+        op = getattr(getattr(torch.ops, namespace), _FIT_BACKWARD_OP[name])
+        torch.library.register_autograd(f"{namespace}::{name}", functools.partial(backward, op), setup_context=setup,
+                                        lib=lib)
     _libs[key] = lib
     return names

@@ -126,3 +126,32 @@ def test_outputs_without_a_gradient_formula(dtype):
             run()
         peaks.append(torch.cuda.max_memory_allocated() - before)
     assert peaks[1] <= peaks[0] + (1 << 20)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_compiled_step(dtype):
+    """A traced fit step (forward and backward, no break in the graph) gives
+    the eager step's loss and gradients bit for bit, over steps whose dropout
+    seed changes, and is traced twice at most (the second time with the seed
+    as a symbol)."""
+    from torch._dynamo.testing import CompileCounterWithBackend
+
+    torch._dynamo.reset()
+    torch.manual_seed(3)
+    cfg = mb.policy.PolicyConfig(h=64, blocks=2, heads=2, kv_heads=1, dropout=0.2)
+    model = mb.policy.CellPolicy(cfg, dtype=DT[dtype]).cuda()
+    batch = mb.policy.token_batch(mb.engine.random_positions(3, 4, 12, seed=5))
+    played = (batch.kind == mb.policy.EMPTY).long().argmax(1)
+    counter = CompileCounterWithBackend("aot_eager")
+    step = torch.compile(lambda seed: model.loss(batch, played, 0.05, seed=seed), backend=counter, fullgraph=True)
+    for seed in (11, 12, 13, 14):
+        results = []
+        for run in (lambda: model.loss(batch, played, 0.05, seed=seed), lambda: step(seed)):
+            model.zero_grad(set_to_none=True)
+            loss = run()
+            loss.backward()
+            results.append([loss.detach(), *(t.grad for t in model.parameters() if t is not model.embed.weight)])
+        for x, y in zip(*results):
+            assert torch.equal(x, y)
+    assert counter.frame_count <= 2
+    mb._lib.check_device_error()
