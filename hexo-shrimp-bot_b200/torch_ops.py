@@ -440,6 +440,24 @@ def _bw_log_probs(op, ctx, g_logp, g_entropy, g_lse, g_top, g_top_logp):
     return op(*ctx.saved_tensors, *grads), None, None, None
 
 
+# Second derivatives: dropout's gradient is linear in its argument, with the
+# forward's mask; the others have no formula, and say so where one is asked
+# for rather than stand as constants.
+def _save_dropout_backward(ctx, inputs, output):
+    grad, ctx.p, ctx.seed, ctx.offset, _ = inputs
+    ctx.grad_dtype = grad.dtype
+
+
+def _bw_dropout_backward(op, ctx, g):
+    return op(g, ctx.p, ctx.seed, ctx.offset, ctx.grad_dtype), None, None, None, None
+
+
+def _no_second(name):
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{name} has no second derivative")
+    return backward
+
+
 _FIT_AUTOGRAD = {"bucket_attention": (_bw_bucket_attention, _save_bucket_attention),
                  "dropout_add": (_bw_dropout_add, _save_dropout_add),
                  "log_probs": (_bw_log_probs, _save_log_probs)}
@@ -450,7 +468,8 @@ _FIT_BACKWARD_OP = {"bucket_attention": "bucket_attention_backward", "dropout_ad
 def define_fit(namespace: str = "mantis_b200") -> list[str]:
     """Define the fit operators in ``namespace`` with this library's CUDA
     kernels, fakes and autograd; their backward passes are ops with fakes too, so
-    a training step traces. ``bucket_attention`` returns (out, lse, full):
+    a training step traces. Second derivatives: dropout has them, the other two
+    raise where one is asked for. ``bucket_attention`` returns (out, lse, full):
     the log-sum-exp and the unrounded output are kept for the backward pass
     and are not differentiable (``requires_grad`` is False), nor is
     ``log_probs``'s lse (its logp, entropy and top_logp are). Returns the
@@ -468,5 +487,10 @@ def define_fit(namespace: str = "mantis_b200") -> list[str]:
         op = getattr(getattr(torch.ops, namespace), _FIT_BACKWARD_OP[name])
         torch.library.register_autograd(f"{namespace}::{name}", functools.partial(backward, op), setup_context=setup,
                                         lib=lib)
+        if name == "dropout_add":
+            torch.library.register_autograd(f"{namespace}::dropout_backward", functools.partial(_bw_dropout_backward, op),
+                                            setup_context=_save_dropout_backward, lib=lib)
+        else:
+            torch.library.register_autograd(f"{namespace}::{_FIT_BACKWARD_OP[name]}", _no_second(name), lib=lib)
     _libs[key] = lib
     return names

@@ -155,3 +155,30 @@ def test_compiled_step(dtype):
             assert torch.equal(x, y)
     assert counter.frame_count <= 2
     mb._lib.check_device_error()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_second_derivatives(dtype):
+    """First gradients are the same with and without create_graph. Through
+    attention and log probabilities a second one raises; dropout's, of a
+    function quadratic in y, is the mask and gain twice."""
+    args = _attention_inputs(1, 2, 1, 9, 32, dtype)
+    seg = _segment_inputs(dtype)
+    for run, xs in ((lambda: fit.bucket_attention(*args)[0].float().sum(), args[:4]),
+                    (lambda: fit.log_probs(*seg)[0].sum(), seg[:1]),
+                    (lambda: fit.log_probs(*seg)[1].square().sum(), seg[:1])):
+        plain = torch.autograd.grad(run(), xs)
+        grads = torch.autograd.grad(run(), xs, create_graph=True)
+        assert all(torch.equal(a, b) and b.requires_grad for a, b in zip(plain, grads))
+        with pytest.raises(RuntimeError, match="second derivative"):
+            torch.autograd.grad(sum(x.float().square().sum() for x in grads), xs[0])
+        loss = run() + 0.1 * sum(x.float().square().sum() for x in grads)  # a penalty beside a loss
+        with pytest.raises(RuntimeError, match="second derivative"):
+            torch.autograd.grad(loss, xs[0])
+    x = torch.randn(6, 40, device=DEV)
+    y = torch.randn(6, 40, device=DEV).to(DT[dtype]).requires_grad_()
+    out = fit.dropout_add(x, y, 0.5, 7, 3)
+    (dy,) = torch.autograd.grad((0.5 * (out - x).square()).sum(), y, create_graph=True)
+    (ddy,) = torch.autograd.grad(dy.float().sum(), y)
+    keep = (out.detach() != x).to(ddy.dtype)
+    assert torch.equal(ddy, 4 * keep)  # a gain of 2, twice: exact
