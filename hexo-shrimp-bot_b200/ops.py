@@ -1296,7 +1296,8 @@ def log_probs(logits, offsets, ranks=None, top=0):
     if not 0 <= top <= 32:
         raise ValueError(f"top must be in [0, 32], got {top}")
     dev = logits.device
-    logp, entropy, lse = torch.empty((3, p), dtype=torch.float32, device=dev).unbind()
+    # tensors of their own: outputs of an op may not share memory
+    logp, entropy, lse = (torch.empty(p, dtype=torch.float32, device=dev) for _ in range(3))
     ti = torch.empty(p, top, dtype=_I64, device=dev)
     tv = torch.empty(p, top, dtype=torch.float32, device=dev)
     call("mb_log_probs", logits.data_ptr(), dtype_code(logits.dtype), logits.shape[0], offsets.data_ptr(), p,

@@ -182,3 +182,33 @@ def test_second_derivatives(dtype):
     (ddy,) = torch.autograd.grad(dy.float().sum(), y)
     keep = (out.detach() != x).to(ddy.dtype)
     assert torch.equal(ddy, 4 * keep)  # a gain of 2, twice: exact
+
+
+def test_log_probs_outputs_share_no_memory():
+    """An in-place step on one output leaves the others and the gradient right."""
+    x, off, ranks, top = _segment_inputs("f32")
+    logp, entropy, lse, *_ = fit.log_probs(x, off, ranks, top)
+    assert len({t.untyped_storage().data_ptr() for t in (logp, entropy, lse)}) == 3
+    kept = entropy.detach().clone(), lse.clone()
+    (want,) = torch.autograd.grad(3 * logp.sum(), x, retain_graph=True)
+    logp *= 3
+    (got,) = torch.autograd.grad(logp.sum(), x)
+    assert torch.equal(got, want) and torch.equal(entropy, kept[0]) and torch.equal(lse, kept[1])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_ops_keep_the_custom_op_contract(dtype):
+    """Schemas (no mutation, no aliasing), autograd keys and fakes, by torch's own check."""
+    which = ("test_schema", "test_autograd_registration", "test_faketensor")
+    args = _attention_inputs(2, 4, 2, 9, 32, dtype, valid=torch.tensor([9, 4], dtype=torch.int32, device=DEV))
+    seg = _segment_inputs(dtype)
+    y = torch.randn(3, 8, device=DEV).to(DT[dtype])
+    out, lse, full = (t.detach() for t in fit.bucket_attention(*args))
+    logp, entropy, seg_lse, tops, top_logp = (t.detach() for t in fit.log_probs(*seg))
+    flat = [t.detach() for t in args]
+    for op, a in ((fit.bucket_attention, args), (fit.log_probs, seg),
+                  (fit.dropout_add, (y.float().requires_grad_(), y.clone().requires_grad_(), 0.3, 5, 6)),
+                  (fit.bucket_attention_backward, (*flat, out, lse, full, out, None, True)),
+                  (fit.log_probs_backward, (seg[0].detach(), *seg[1:3], seg_lse, entropy, tops, logp, entropy, top_logp)),
+                  (fit.dropout_backward, (y, 0.3, 5, 6, torch.float32))):
+        torch.library.opcheck(op.default, a, test_utils=which)
