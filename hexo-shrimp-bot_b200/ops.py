@@ -1311,15 +1311,19 @@ def log_probs_backward(logits, offsets, ranks, got, g_logp=None, g_entropy=None,
     entropy) + sum(g_top * top_logp), from ``log_probs``'s result ``got``; each
     gradient is fp32 of its output's shape, or None for zero."""
     p = _segments(logits, offsets, ranks)
-    top = 0 if g_top is None else got.top.shape[1]
-    for g, like, name in ((g_logp, got.logp, "g_logp"), (g_entropy, got.entropy, "g_entropy"),
-                          (g_top, got.top_logp, "g_top")):
+    # the kernel reads these of the forward's result
+    for t, dim, dtype in ((got.lse, 1, torch.float32), (got.entropy, 1, torch.float32), (got.top, 2, _I64)):
+        if not t.is_cuda or t.dtype != dtype or t.dim() != dim or t.shape[0] != p or not t.is_contiguous():
+            raise ValueError("got must be the result of log_probs on the same segments")
+    shape = got.top.shape
+    if shape[1] > 32:
+        raise ValueError("got must be the result of log_probs on the same segments")
+    for g, want, name in ((g_logp, (p,), "g_logp"), (g_entropy, (p,), "g_entropy"), (g_top, shape, "g_top")):
         if g is not None:
             _cuda(g)
-            if g.dtype != torch.float32 or g.shape != like.shape or not g.is_contiguous():
+            if g.dtype != torch.float32 or g.shape != want or not g.is_contiguous():
                 raise ValueError(f"{name} must be a contiguous fp32 tensor of its output's shape")
-    if got.lse.shape != (p,):
-        raise ValueError("got must be the result of log_probs on the same segments")
+    top = 0 if g_top is None else shape[1]
     grad = torch.empty(logits.shape[0] + 8, dtype=logits.dtype, device=logits.device)
     skip = (logits.data_ptr() % 16) // logits.element_size()  # aligned as the logits are
     grad = grad[skip:skip + logits.shape[0]]

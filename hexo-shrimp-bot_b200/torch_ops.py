@@ -359,7 +359,7 @@ def _fit_log_probs(logits, offsets, ranks, top=0):
 
 
 def _fit_log_probs_backward(logits, offsets, ranks, lse, entropy, top, g_logp, g_entropy, g_top_logp):
-    got = ops.LogProbs(lse, entropy, lse, top, top)  # of its values the kernel reads lse, entropy and top
+    got = ops.LogProbs(None, entropy, lse, top, None)  # what the kernel reads
     return ops.log_probs_backward(logits, offsets, ranks, got, g_logp, g_entropy, g_top_logp)
 
 

@@ -212,3 +212,23 @@ def test_ops_keep_the_custom_op_contract(dtype):
                   (fit.log_probs_backward, (seg[0].detach(), *seg[1:3], seg_lse, entropy, tops, logp, entropy, top_logp)),
                   (fit.dropout_backward, (y, 0.3, 5, 6, torch.float32))):
         torch.library.opcheck(op.default, a, test_utils=which)
+
+
+def test_log_probs_backward_refuses_another_result():
+    """A result on the host, of another type or of other segments is refused
+    before any launch."""
+    x, off, ranks, top = _segment_inputs("f32")
+    x = x.detach()
+    got = ops.log_probs(x, off, ranks, top=top)
+    g = torch.ones(2, device=DEV)
+    short = ops.log_probs(x, off[:2], ranks[:1], top=top)
+    wide = torch.zeros(2, 4, dtype=torch.int64, device=DEV)
+    for bad in (got._replace(lse=got.lse.cpu()), got._replace(entropy=got.entropy.cpu()),
+                got._replace(top=got.top.cpu()), got._replace(lse=got.lse.double()),
+                got._replace(entropy=got.entropy.bfloat16()), got._replace(entropy=short.entropy),
+                got._replace(top=got.top.int()), got._replace(top=short.top), got._replace(top=got.top[:, 0]),
+                got._replace(top=wide[:, ::2]), got._replace(top=torch.zeros(2, 33, dtype=torch.int64, device=DEV))):
+        with pytest.raises(ValueError, match="result of log_probs"):
+            ops.log_probs_backward(x, off, ranks, bad, g)
+    with pytest.raises(ValueError, match="g_top"):
+        ops.log_probs_backward(x, off, ranks, got, g, None, torch.ones(2, 3, device=DEV))
