@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from golden_io import mb
+from test_gpu_fit_ops import _bounds, _case
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -232,3 +233,58 @@ def test_log_probs_backward_refuses_another_result():
             ops.log_probs_backward(x, off, ranks, bad, g)
     with pytest.raises(ValueError, match="g_top"):
         ops.log_probs_backward(x, off, ranks, got, g, None, torch.ones(2, 3, device=DEV))
+
+
+# ------------------------------------------------- attention's other forms
+def _to_device(args):
+    """q, k, v as views of one fused tensor, then go and the rest, on the device."""
+    q, k, v, go, *rest = args
+    fused = torch.cat([q, k, v], 1).permute(0, 2, 1, 3).contiguous().to(DEV).permute(0, 2, 1, 3)
+    return (*fused.split([q.shape[1], k.shape[1], k.shape[1]], 1), go.to(DEV),
+            *(x.to(DEV) if x is not None else None for x in rest))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [16, 32, 64, 128])
+@pytest.mark.parametrize("length,layout,ragged", [(1, "hex", False), (37, "hex", False), (129, "causal", True),
+                                                  (200, "hex", True), (257, "line", True), (513, "line", False),
+                                                  (1100, "line", False)])
+def test_attention_serving_form(dtype, d, length, layout, ragged):
+    """The form that keeps nothing for a backward pass, elementwise against the
+    oracle: its bound has the probabilities' and the output's roundings to
+    bf16, and no more."""
+    args = _case(1 if length > 500 else 3, 4, 2, length, d, dtype, layout, ragged=ragged, seed=130)
+    (want, want_lse, *_), (bound, bound_lse, *_) = _bounds(*args, dtype)
+    q, k, v, _, *rest = _to_device(args)
+    out, lse = ops.bucket_attention(q, k, v, *rest, with_lse=True)
+    for name, x, y, b in (("out", out, want, bound), ("lse", lse, want_lse, bound_lse)):
+        x = x.double().cpu()
+        fin = torch.isfinite(y)
+        assert torch.equal(fin, torch.isfinite(x)) and torch.equal(x[~fin], y[~fin]), name
+        over = ((x - y).abs() - b)[fin]
+        assert over.numel() == 0 or float(over.max()) <= 1e-12, f"{name}: {float(over.max()):.3e} over its bound"
+    mb._lib.check_device_error()
+
+
+def _within(name, got, want, bound):
+    got = got.detach().double().cpu()
+    over = (got - want).abs() - bound
+    assert got.shape == want.shape
+    assert over.numel() == 0 or float(over.max()) <= 1e-12, f"{name}: {float(over.max()):.3e} over its bound"
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("bias_grad", [True, False])
+@pytest.mark.parametrize("heads,kv,length,d", [(4, 4, 70, 32), (4, 1, 140, 64)])
+def test_attention_autograd_matches_the_oracle(dtype, bias_grad, heads, kv, length, d):
+    """The torch op's gradients, from strided views and a gradient in another layout."""
+    args = _case(3, heads, kv, length, d, dtype, ragged=True, seed=131)
+    want, bound = _bounds(*args, dtype)
+    q, k, v, go, bias, *rest = _to_device(args)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)] + [bias.requires_grad_(bias_grad)]
+    out, lse, _ = fit.bucket_attention(*leaves, *rest)
+    grads = torch.autograd.grad(out, leaves if bias_grad else leaves[:3], go)
+    for name, x, y, b in zip(("out", "dq", "dk", "dv", "dbias"), (out, *grads), (want[0], *want[2:]),
+                             (bound[0], *bound[2:])):
+        _within(name, x, y, b)
+    mb._lib.check_device_error()
