@@ -72,6 +72,7 @@ SIGNATURES = {
     "mb_gemm_set_plan": "ii",
     "mb_bucket_attention": "pppiliiillllllllllfpipiiplpplllppp",
     "mb_bucket_attention_workspace": "iliiilip",
+    "mb_bucket_attention_limit_parts": "l",
     "mb_bucket_attention_backward": "pppiliiillllllllllfpipiiplpplllppplllplppppp",
     "mb_dropout_add": "pilpillllfllpilp",
     "mb_log_probs": "pilplpipppppp",

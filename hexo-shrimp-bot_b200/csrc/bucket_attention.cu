@@ -485,6 +485,12 @@ inline int bias_sum(const Args& a, int64_t ctas, cudaStream_t s) {
   return launch_status("bucket_attention_backward");
 }
 
+// The dQ and dK / dV parts, delta, then the bias sums of each CTA.
+inline int64_t workspace_bytes(const BackwardPlan& plan, int64_t n_pos, int heads, int64_t length, int n_buckets) {
+  const int64_t ctas = std::max(n_pos * cdiv(length, TQ), plan.ctas);
+  return 4 * (plan.dq_words + plan.dkv_words + n_pos * heads * length + ctas * heads * n_buckets);
+}
+
 inline int check(const Args& a, int dtype, const char* what) {
   MB_REQUIRE(valid_dtype(dtype), "%s: bad dtype", what);
   MB_REQUIRE(a.n_pos >= 0 && a.length >= 0 && a.heads > 0 && a.kv_heads > 0 && a.heads % a.kv_heads == 0,
@@ -541,16 +547,20 @@ int mb_bucket_attention(const void* q, const void* k, const void* v, int dtype, 
   return MB_BUCKET_DISPATCH(dtype, head_dim, bucket::simt_forward, a, s);
 }
 
+int mb_bucket_attention_limit_parts(int64_t bytes) {
+  MB_REQUIRE(bytes >= 0, "bucket_attention_limit_parts: negative size");
+  bucket::part_limit.store(bytes / 4 + (bytes % 4 != 0), std::memory_order_relaxed);
+  return MB_OK;
+}
+
 int mb_bucket_attention_workspace(int dtype, int64_t n_pos, int heads, int kv_heads, int head_dim, int64_t length,
                                   int n_buckets, int64_t* bytes) {
   MB_REQUIRE(bytes, "bucket_attention_workspace: null pointer");
   MB_REQUIRE(valid_dtype(dtype) && n_pos >= 0 && heads > 0 && kv_heads > 0 && head_dim > 0 && length >= 0 &&
                  n_buckets > 0,
              "bucket_attention_workspace: bad sizes");
-  // the dQ and dK / dV parts, delta, then the bias sums of each CTA
-  const bucket::BackwardPlan plan = bucket::backward_plan(n_pos, heads, kv_heads, head_dim, length, dtype);
-  const int64_t ctas = std::max(n_pos * cdiv(length, bucket::TQ), plan.ctas);
-  *bytes = 4 * (plan.dq_words + plan.dkv_words + n_pos * heads * length + ctas * heads * n_buckets);
+  *bytes = bucket::workspace_bytes(bucket::backward_plan(n_pos, heads, kv_heads, head_dim, length, dtype), n_pos, heads,
+                                   length, n_buckets);
   return MB_OK;
 }
 
@@ -581,18 +591,18 @@ int mb_bucket_attention_backward(const void* q, const void* k, const void* v, in
   }
   MB_REQUIRE(q && k && v && bias && bucket_map && coords && out && lse && grad_out && workspace && dq && dk && dv,
              "bucket_attention_backward: null pointer");
-  int64_t need = 0;
-  if (int rc = mb_bucket_attention_workspace(dtype, n_pos, heads, kv_heads, head_dim, length, n_buckets, &need)) return rc;
+  // one plan for the whole call: the limit on parts may change beside it
+  const bucket::BackwardPlan plan = bucket::backward_plan(n_pos, heads, kv_heads, head_dim, length, dtype);
+  const int64_t need = bucket::workspace_bytes(plan, n_pos, heads, length, n_buckets);
   MB_REQUIRE(workspace_bytes >= need && aligned(workspace, 16),
              "bucket_attention_backward: the workspace needs %lld bytes, 16-byte aligned", (long long)need);
-  const bucket::BackwardPlan plan = bucket::backward_plan(n_pos, heads, kv_heads, head_dim, length, dtype);
   a.dq_part = (float*)workspace;
   a.dkv_part = a.dq_part + plan.dq_words;
   a.delta = a.dkv_part + plan.dkv_words;
   a.bias_part = a.delta + n_pos * heads * length;
   int64_t parts = n_pos * cdiv(length, bucket::TQ);  // of a bias sum
   if (bucket::tc_serves(a, dtype)) {
-    if (int rc = bucket::tc_backward(a, s)) return rc;
+    if (int rc = bucket::tc_backward(a, plan, s)) return rc;
     parts = plan.ctas;
   } else {
     if (int rc = MB_BUCKET_DISPATCH(dtype, head_dim, bucket::simt_backward, a, s)) return rc;

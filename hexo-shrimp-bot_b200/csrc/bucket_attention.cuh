@@ -10,6 +10,8 @@
 // radii; a row without a key (or past valid[p]) has out = 0, lse = -inf.
 #pragma once
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace mb {
@@ -134,8 +136,6 @@ int configure(K kern, size_t bytes, const char* what) {
 // The tensor-core forms (bucket_attention_sm100.cu).
 bool tc_serves(const Args& a, int dtype);
 int tc_forward(const Args& a, cudaStream_t s);
-int tc_backward(const Args& a, cudaStream_t s);
-
 // How the tensor-core backward pass is shared (see bucket_attention_sm100.cu):
 // by whole items, or key tiles, how many of them a launch takes (their dQ parts
 // are kept together) and the CTAs that share a key tile's queries.
@@ -146,6 +146,10 @@ struct BackwardPlan {
   int64_t dq_words, dkv_words;  // fp32 workspace words of the parts
 };
 BackwardPlan backward_plan(int64_t n_pos, int heads, int kv_heads, int head_dim, int64_t length, int dtype);
+int tc_backward(const Args& a, const BackwardPlan& plan, cudaStream_t s);
+
+// fp32 words of dQ parts that a caller allows a backward pass (0: the default).
+extern std::atomic<int64_t> part_limit;
 
 }  // namespace bucket
 }  // namespace mb

@@ -1226,11 +1226,10 @@ int launch_forward(const Args& a, cudaStream_t s) {
 }
 
 template <int D>
-int launch_backward(const Args& args, cudaStream_t s) {
+int launch_backward(const Args& args, const BackwardPlan& plan, cudaStream_t s) {
   Args a = args;
   const int64_t tiles = cdiv(a.length, BK), n = a.n_pos * a.heads * a.length * D;
   const size_t smem = backward_smem<D>(a);
-  const BackwardPlan plan = backward_plan(a.n_pos, a.heads, a.kv_heads, D, a.length, MB_BF16);
   delta_kernel<D><<<(unsigned)cdiv(n / 8, 256), 256, 0, s>>>(a);
   if (plan.whole) {
     auto kern = backward_kernel<D, true>;
@@ -1279,16 +1278,24 @@ int tc_forward(const Args& a, cudaStream_t s) {
                        : tc::launch_forward<128>(a, s);
 }
 
-int tc_backward(const Args& a, cudaStream_t s) {
-  return a.dim == 32   ? tc::launch_backward<32>(a, s)
-         : a.dim == 64 ? tc::launch_backward<64>(a, s)
-                       : tc::launch_backward<128>(a, s);
+int tc_backward(const Args& a, const BackwardPlan& plan, cudaStream_t s) {
+  return a.dim == 32   ? tc::launch_backward<32>(a, plan, s)
+         : a.dim == 64 ? tc::launch_backward<64>(a, plan, s)
+                       : tc::launch_backward<128>(a, plan, s);
 }
 
+std::atomic<int64_t> part_limit{0};
+
 // Whole items where every CTA of one round (two per SM) has two of them or
-// more. Else a launch takes as many key tiles as 2 GiB of dQ parts hold (four
-// at least), and where it has fewer than two rounds of CTAs, a key tile's
-// queries are shared by up to 16 CTAs of four steps or more.
+// more. Else a launch takes as many key tiles as 2 GiB of dQ parts hold, but
+// four (each launch fills the GPU, and the running sum passes through memory
+// once for four parts) as long as those and the running sum stay within 16 GiB;
+// beyond that fewer, one at least. 147 positions x 16 heads on 4 x 4,096 x 128,
+// a part of 4.6 GiB: four tiles 173 ms and 26.5 GiB, two (taken) 187 ms and
+// 17.3 GiB, one 217 ms and 12.7 GiB, whole items 178 ms and 8.1 GiB, but 114
+// against 78 ms for four where the lengths differ. A caller's limit holds
+// alone. Where a launch has fewer than two rounds of CTAs, a key tile's queries
+// are shared by up to 16 CTAs of four steps or more.
 BackwardPlan backward_plan(int64_t n_pos, int heads, int kv_heads, int head_dim, int64_t length, int dtype) {
   BackwardPlan p = {};
   if (dtype != MB_BF16 || head_dim == 16) return p;  // the CUDA-core kernels keep no parts
@@ -1296,7 +1303,9 @@ BackwardPlan backward_plan(int64_t n_pos, int heads, int kv_heads, int head_dim,
   p.tiles = cdiv(length, tc::BK);
   const int64_t n = std::max<int64_t>(n_pos * heads * length * head_dim, 1);
   p.whole = n_pos * kv_heads >= 2 * round;
-  p.chunk = std::min(p.tiles, std::max<int64_t>(4, (int64_t(1) << 29) / n));
+  const int64_t limit = part_limit.load(std::memory_order_relaxed);
+  const int64_t least = limit ? 1 : std::clamp<int64_t>((int64_t(1) << 32) / n - 1, 1, 4);
+  p.chunk = std::min(p.tiles, std::max(least, (limit ? limit : int64_t(1) << 29) / n));
   const int64_t ctas = n_pos * kv_heads * p.chunk, steps = heads / kv_heads * cdiv(length, tc::BQ);
   p.split = 1;
   while (!p.whole && p.split < 16 && ctas * p.split < 2 * round && steps / (2 * p.split) >= 4) p.split *= 2;

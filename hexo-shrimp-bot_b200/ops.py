@@ -1180,6 +1180,15 @@ def _bucket_workspace(*sizes) -> int:
     return need.value
 
 
+def bucket_attention_limit_parts(limit: int = 0) -> None:
+    """Limit the parts of dq that ``bucket_attention_backward`` keeps in its
+    workspace to ``limit`` bytes (0: the default, 2 GiB, or four key tiles'
+    within 16 GiB). A part is an fp32 tensor of q's size; one and the running sum
+    are kept in any case, and fewer at a time take longer. Process-wide."""
+    call("mb_bucket_attention_limit_parts", int(limit))
+    _bucket_workspace.cache_clear()
+
+
 def bucket_attention_backward(q, k, v, bias, bucket_map, coords, valid, out, stats, grad_out, scale=None,
                               bias_grad=True):
     """Gradients of ``bucket_attention`` from its output, its

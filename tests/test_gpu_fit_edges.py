@@ -288,3 +288,27 @@ def test_attention_autograd_matches_the_oracle(dtype, bias_grad, heads, kv, leng
                              (bound[0], *bound[2:])):
         _within(name, x, y, b)
     mb._lib.check_device_error()
+
+
+@pytest.mark.parametrize("d,heads,kv", [(32, 2, 2), (64, 4, 1), (128, 2, 1)])
+@pytest.mark.parametrize("parts", [1, 2, 4, 5, 6])
+def test_attention_gradients_in_chunks_of_key_tiles(d, heads, kv, parts):
+    """Six key tiles, `parts` of dQ kept at a time: the running sum over
+    chunks, a last chunk of fewer tiles, and positions that end in the first
+    chunk, against the oracle; the same again bit for bit."""
+    length = 700
+    args = list(_case(3, heads, kv, length, d, "bf16", "line", seed=140))
+    args[-1] = torch.tensor([700, 130, 391], dtype=torch.int32)
+    want, bound = _bounds(*args, "bf16")
+    q, k, v, go, *rest = _to_device(args)
+    try:
+        ops.bucket_attention_limit_parts(parts * 4 * 3 * heads * length * d)
+        out, st = ops.bucket_attention(q, k, v, *rest, for_backward=True)
+        grads = ops.bucket_attention_backward(q, k, v, *rest, out, st, go)
+        again = ops.bucket_attention_backward(q, k, v, *rest, out, st, go)
+    finally:
+        ops.bucket_attention_limit_parts(0)
+    for name, x, x2, y, b in zip(("dq", "dk", "dv", "dbias"), grads, again, want[2:], bound[2:]):
+        _within(name, x, y, b)
+        assert torch.equal(x, x2)
+    mb._lib.check_device_error()
