@@ -1291,8 +1291,8 @@ std::atomic<int64_t> part_limit{0};
 // four (each launch fills the GPU, and the running sum passes through memory
 // once for four parts) as long as those and the running sum stay within 16 GiB;
 // beyond that fewer, one at least. 147 positions x 16 heads on 4 x 4,096 x 128,
-// a part of 4.6 GiB: four tiles 173 ms and 26.5 GiB, two (taken) 187 ms and
-// 17.3 GiB, one 217 ms and 12.7 GiB, whole items 178 ms and 8.1 GiB, but 114
+// a part of 4.6 GiB: four tiles 173 ms and 23.0 GiB, two (taken) 187 ms and
+// 13.8 GiB, one 217 ms and 9.2 GiB, whole items 178 ms and 4.7 GiB, but 114
 // against 78 ms for four where the lengths differ. A caller's limit holds
 // alone. Where a launch has fewer than two rounds of CTAs, a key tile's queries
 // are shared by up to 16 CTAs of four steps or more.

@@ -70,3 +70,15 @@ def test_limit_on_parts(limit):
     assert wrapped() == default
     with pytest.raises(ValueError, match="negative"):
         limit(-1)
+
+
+def test_bias_sums_of_the_path_that_runs():
+    """The tensor cores keep bias sums for 296 CTAs, not one for each of 70,000
+    query tiles; the CUDA cores, which keep no parts, have theirs in the same place."""
+    size = 10_000, 16, 16, 32, 400
+    parts, delta = _part(10_000, 16, 400, 32), 4 * 10_000 * 16 * 400
+    assert _bytes(BF16, *size, 128) == parts + delta + 4 * 296 * 16 * 128
+    sums = 4 * 10_000 * 7 * 16 * 128
+    assert _bytes(F32, *size, 128) == delta + sums
+    # one key tile of a bf16 batch has no parts: the CUDA cores' sums decide
+    assert _bytes(BF16, 10_000, 16, 16, 32, 40, 128) == 4 * 10_000 * 16 * (40 + 128)

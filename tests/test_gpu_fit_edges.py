@@ -13,7 +13,7 @@ from test_gpu_fit_ops import _bounds, _case
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
-ops = mb.ops
+ops, _lib = mb.ops, mb._lib
 DT = {"f32": torch.float32, "bf16": torch.bfloat16}
 
 
@@ -311,4 +311,34 @@ def test_attention_gradients_in_chunks_of_key_tiles(d, heads, kv, parts):
     for name, x, x2, y, b in zip(("dq", "dk", "dv", "dbias"), grads, again, want[2:], bound[2:]):
         _within(name, x, y, b)
         assert torch.equal(x, x2)
+    mb._lib.check_device_error()
+
+
+@pytest.mark.parametrize("dtype,d,p,length", [("bf16", 32, 3, 300), ("bf16", 64, 40, 70), ("bf16", 16, 3, 150),
+                                              ("f32", 32, 3, 150)])
+def test_attention_gradients_within_their_workspace(dtype, d, p, length):
+    """Through the C entry with the workspace that it asks for and not a byte
+    more, on rows of 16 bytes and off them (the CUDA cores, with the bias sums
+    where the tensor cores keep their parts): the same gradients as the wrapper's
+    to the roundings between the two paths, and the bytes behind it untouched."""
+    args = _case(p, 4, 2, length, d, dtype, ragged=True, seed=150)
+    want, bound = _bounds(*args, dtype)
+    q, k, v, go, bias, bmap, coords, valid = _to_device(args)
+    wide = [torch.empty(*t.shape[:3], d + 1, dtype=t.dtype, device=DEV)[..., 1:] for t in (q, k, v)]
+    for w, t in zip(wide, (q, k, v)):
+        w.copy_(t)
+    for q, k, v in ((q, k, v), wide):
+        out, st = ops.bucket_attention(q, k, v, bias, bmap, coords, valid, for_backward=True)
+        kept, fixed = ops._bucket_args(q, k, v, bias, bmap, coords, valid, None)
+        need = ops._bucket_workspace(_lib.dtype_code(q.dtype), p, 4, 2, d, length, bias.shape[0])
+        ws = torch.full((need + 4096,), 0xA5, dtype=torch.uint8, device=DEV)
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=DEV) for t in (q, k, v))
+        dbias = torch.empty_like(bias)
+        g = go.contiguous()
+        _lib.call("mb_bucket_attention_backward", *fixed, out.data_ptr(), *out.stride()[:3], _lib.ptr(st.full),
+                  st.lse.data_ptr(), g.data_ptr(), *g.stride()[:3], ws.data_ptr(), need, dq.data_ptr(), dk.data_ptr(),
+                  dv.data_ptr(), dbias.data_ptr(), _lib.stream_of(q.device))
+        for name, x, y, b in zip(("dq", "dk", "dv", "dbias"), (dq, dk, dv, dbias), want[2:], bound[2:]):
+            _within(name, x, y, b)
+        assert bool((ws[need:] == 0xA5).all())
     mb._lib.check_device_error()
