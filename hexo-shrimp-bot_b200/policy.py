@@ -103,7 +103,8 @@ class CellPolicy(nn.Module):
         drop = cfg.dropout if self.training else 0.0
         x = self.embed(batch.kind)
         for i, block in enumerate(self.blocks):
-            qkv = self._linear(block.qkv, block.ln_attn(x)).view(p, length, cfg.heads + 2 * cfg.kv_heads, -1)
+            qkv = self._linear(block.qkv, block.ln_attn(x)).view(p, length, cfg.heads + 2 * cfg.kv_heads,
+                                                                 cfg.h // cfg.heads)
             q, k, v = qkv.permute(0, 2, 1, 3).split([cfg.heads, cfg.kv_heads, cfg.kv_heads], 1)
             where = (self.bucket_map, batch.coords, batch.valid)
             if torch.is_grad_enabled():
