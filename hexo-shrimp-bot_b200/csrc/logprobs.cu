@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(kMaxThreads, TOP ? 4 : 6) forward_kernel(
 // last segment clear what lies outside all offsets. Off the ordinary path: every
 // step here reads the offsets, and no element is cleared twice.
 template <typename T>
-__device__ __noinline__ void zero_malformed(const int64_t* __restrict__ offsets, int64_t n_segments, int64_t p,
+__device__ __forceinline__ void zero_malformed(const int64_t* __restrict__ offsets, int64_t n_segments, int64_t p,
                                             int64_t n, T* __restrict__ grad) {
   __shared__ long long reach, next;
   const long long end = min(max(offsets[p + 1], (int64_t)0), n);

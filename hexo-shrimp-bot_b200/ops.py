@@ -1306,7 +1306,8 @@ def log_probs(logits, offsets, ranks=None, top=0):
         raise ValueError(f"top must be in [0, 32], got {top}")
     dev = logits.device
     # tensors of their own: outputs of an op may not share memory
-    logp, entropy, lse = (torch.empty(p, dtype=torch.float32, device=dev) for _ in range(3))
+    logp = torch.empty(p, dtype=torch.float32, device=dev)
+    entropy, lse = torch.empty_like(logp), torch.empty_like(logp)
     ti = torch.empty(p, top, dtype=_I64, device=dev)
     tv = torch.empty(p, top, dtype=torch.float32, device=dev)
     call("mb_log_probs", logits.data_ptr(), dtype_code(logits.dtype), logits.shape[0], offsets.data_ptr(), p,
@@ -1320,12 +1321,12 @@ def log_probs_backward(logits, offsets, ranks, got, g_logp=None, g_entropy=None,
     entropy) + sum(g_top * top_logp), from ``log_probs``'s result ``got``; each
     gradient is fp32 of its output's shape, or None for zero."""
     p = _segments(logits, offsets, ranks)
-    # the kernel reads these of the forward's result
-    for t, dim, dtype in ((got.lse, 1, torch.float32), (got.entropy, 1, torch.float32), (got.top, 2, _I64)):
-        if not t.is_cuda or t.dtype != dtype or t.dim() != dim or t.shape[0] != p or not t.is_contiguous():
-            raise ValueError("got must be the result of log_probs on the same segments")
-    shape = got.top.shape
-    if shape[1] > 32:
+    lse, entropy, tops = got.lse, got.entropy, got.top  # what the kernel reads of the forward's result
+    shape = tops.shape
+    if not (lse.shape == entropy.shape == (p,) and len(shape) == 2 and shape[0] == p and shape[1] <= 32
+            and lse.dtype == entropy.dtype == torch.float32 and tops.dtype == _I64
+            and lse.is_cuda and entropy.is_cuda and tops.is_cuda
+            and lse.is_contiguous() and entropy.is_contiguous() and tops.is_contiguous()):
         raise ValueError("got must be the result of log_probs on the same segments")
     for g, want, name in ((g_logp, (p,), "g_logp"), (g_entropy, (p,), "g_entropy"), (g_top, shape, "g_top")):
         if g is not None:
@@ -1337,6 +1338,6 @@ def log_probs_backward(logits, offsets, ranks, got, g_logp=None, g_entropy=None,
     skip = (logits.data_ptr() % 16) // logits.element_size()  # aligned as the logits are
     grad = grad[skip:skip + logits.shape[0]]
     call("mb_log_probs_backward", ptr(logits), dtype_code(logits.dtype), logits.shape[0], ptr(offsets), p, ptr(ranks),
-         top, ptr(got.lse), ptr(got.entropy), ptr(got.top), ptr(g_logp), ptr(g_entropy), ptr(g_top), ptr(grad),
+         top, lse.data_ptr(), entropy.data_ptr(), tops.data_ptr(), ptr(g_logp), ptr(g_entropy), ptr(g_top), ptr(grad),
          stream_of(logits.device))
     return grad
