@@ -288,17 +288,22 @@ __device__ __forceinline__ int single_entry(const Args& a, const Box& key, const
 // ---------------------------------------------------------------- forward --
 // One CTA of 128 threads per (position, head, 128 queries). A thread owns a
 // query row (its TMEM lane). Key tiles of 32 (head size 32, six CTAs per SM)
-// or 64 (head size 64, four, and 128, two: what TMEM holds; 1,024 x 8 heads of 256
-// tokens take 302 us with 64-key tiles at four CTAs, 315 us with 32 at eight,
-// whose 64 registers spill, 285 us at six): S = Q K^T into
+// or 64 (head size 64, four, and 128, two: what TMEM holds; against this choice
+// 1,024 positions x 8 heads x 32-256 tokens take 6% more with 64-key tiles at four
+// CTAs and 11% more with 32 at eight, whose 64 registers spill): S = Q K^T into
 // TMEM, biased scores and exponentials in registers, P as bf16 back over S,
 // O += P V with P read from TMEM. One commit covers PV(j) and S(j + 1), and
 // K and V of tile j + 1 are copied while tile j's softmax runs. The running
 // maximum that P and O are relative to is raised only when a tile's maximum
 // passes it by 2^8 (O is then rescaled in TMEM), which the final division
-// undoes exactly. For the backward pass (FULL) P is carried as the sum of two
-// bf16 values: delta = dO . out must match sum P dP of the recomputed fp32 P
-// to about 2^-18, or the bias sums, where dS cancels, keep P's 2^-9.
+// undoes exactly. Serving rounds P to bf16 once, the type that the product takes:
+// 2^-9 of each term, next to the output's own 2^-9 (2.3e-3 off 64 bits in all, 1.7e-3
+// for the output's rounding alone). For the backward pass (FULL) P is carried
+// as the sum of two bf16 values: delta = dO . out must match sum P dP of the
+// recomputed fp32 P to about 2^-18, or the bias sums, where dS cancels, keep P's
+// 2^-9. O accumulates in TMEM, which truncates by 2^-24 a step of 16 keys: at 512 k
+// keys the serving form's sums are off by bf16's own half step, and FULL's are
+// flushed every 512 keys.
 //
 // Bound: issue and the latencies around it, not the tensor cores (6% active at
 // head size 32, 23% at 64) nor HBM. 1,024 positions x 8 heads x 32-256 tokens,
@@ -625,7 +630,10 @@ __global__ void __launch_bounds__(kFwdThreads, FwdPlan<D>::CTAS) forward_kernel(
 //   shared memory, and dS added to the bias sums    (registers)
 //   dV += P^T dO, dK += dS^T Q, dQ = dS K           (TMEM)
 // dS^T is written once, rows of queries: as it is it is dK's A operand, and
-// read MN-major it is dQ's. dK and dV stay in TMEM to the tile's end.
+// read MN-major it is dQ's. dK and dV stay in TMEM to the tile's end. P and dS are
+// rounded to bf16 as operands, 2^-9 of each term like the results' own rounding;
+// TMEM truncates dK's and dV's sums by 2^-24 a step of 16 queries, bf16's half step
+// after 512 k queries. The bias sums take dS before its rounding.
 // Bias sums: one private fp32 sum per (bucket, thread) in shared memory,
 // bank = thread, so updates never conflict and every sum has a fixed order.
 //

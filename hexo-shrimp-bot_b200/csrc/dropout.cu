@@ -12,10 +12,10 @@
 // Bound: HBM (x, y read, out written; 10 B an element for an fp32 stream and
 // a bf16 branch), with the generator close behind: one Philox block serves four
 // elements, ten rounds of two wide multiplies and two three-way xors. Eight
-// elements a thread (two blocks, 16- and 32-byte accesses). 262,144 x 256: 97 us
-// forward and 78 us backward in turn, 182 us for the two, 92% of the measured
-// HBM rate (95 and 86 us with 72-76% of issue slots before the round keys were
-// added up on the host).
+// elements a thread (two blocks, 16- and 32-byte accesses). 262,144 x 256 from
+// a cold L2: 104 us forward and 84 us backward; 185 to 190 us for the two in turn,
+// 88 to 90% of the measured HBM rate (the generator took 72-76% of issue slots
+// before the round keys were added up on the host).
 #include "common.cuh"
 
 namespace mb {

@@ -108,7 +108,8 @@ def line_buckets(n_buckets: int = 32, max_distance: int = 128, causal: bool = Fa
     line of tokens (coordinates (t, 0)) for the bucketed-bias attention: on
     each side half the buckets for exact distances, then log-spaced ones up to
     ``max_distance``. ``causal`` excludes later keys (-1) and gives the earlier
-    ones every bucket."""
+    ones every bucket. The log-spaced scheme is that of Raffel et al. (2020,
+    relative position buckets)."""
     side = n_buckets if causal else n_buckets // 2
     exact = side // 2
     if exact < 1 or max_distance <= exact or (not causal and n_buckets % 2):

@@ -1249,7 +1249,9 @@ def dropout_add(x, y, p, seed, offset=0):
     zero), in x's dtype. The keep mask is a function of (seed, offset, row-
     major index) alone, drawn from Philox4x32-10, and never stored:
     ``dropout_backward`` with the same p, seed and offset draws it again.
-    Use another ``offset`` (or seed) for every call of a step."""
+    Use another ``offset`` (or seed) for every call of a step. Both are numbers of
+    the host: a captured CUDA graph draws the mask of its capture at every
+    replay, so capture the parts of a step around it."""
     _cuda(x, y)
     if y.dim() == 0:
         raise ValueError("y must have at least one dimension")

@@ -512,11 +512,6 @@ int mb_bucket_attention(const void* q, const void* k, const void* v, int dtype, 
  * order. workspace: mb_bucket_attention_workspace bytes, 16-byte aligned. */
 int mb_bucket_attention_workspace(int dtype, int64_t n_pos, int heads, int kv_heads, int head_dim, int64_t length,
                                   int n_buckets, int64_t* bytes);
-/* Limits the dQ parts that a backward pass keeps in its workspace to `bytes`
- * (one key tile's part and the running sum are kept in any case; 0: the
- * default, 2 GiB, or four tiles' parts within 16 GiB). Process-wide; a
- * workspace is sized under the limit that its call runs under. */
-int mb_bucket_attention_limit_parts(int64_t bytes);
 int mb_bucket_attention_backward(const void* q, const void* k, const void* v, int dtype, int64_t n_pos, int heads,
                                  int kv_heads, int head_dim, int64_t length, int64_t q_pos, int64_t q_head,
                                  int64_t q_row, int64_t k_pos, int64_t k_head, int64_t k_row, int64_t v_pos,
@@ -526,6 +521,12 @@ int mb_bucket_attention_backward(const void* q, const void* k, const void* v, in
                                  int64_t o_row, const float* full, const float* lse, const void* grad_out,
                                  int64_t g_pos, int64_t g_head, int64_t g_row, void* workspace,
                                  int64_t workspace_bytes, void* dq, void* dk, void* dv, float* dbias, void* stream);
+
+/* Limits the dQ parts that a backward pass keeps in its workspace to `bytes`
+ * (one key tile's part and the running sum are kept in any case; 0: the
+ * default, 2 GiB, or four tiles' parts within 16 GiB). Process-wide; a
+ * workspace is sized under the limit that its call runs under. */
+int mb_bucket_attention_limit_parts(int64_t bytes);
 
 /* Dropout on a residual branch: out[e] = x[e] + (r(e) >= threshold ? y[e] *
  * gain : 0), x NULL reading 0. r(e) is word e % 4 of Philox4x32-10 at counter
