@@ -488,9 +488,10 @@ inline int bias_sum(const Args& a, int64_t ctas, cudaStream_t s) {
 // The workspace's words ahead of delta: on the tensor cores the dQ and dK / dV
 // parts and the bias sums of the plan's CTAs; on the CUDA cores, which serve bf16
 // rows off 16 bytes too, the bias sums of every query tile and no parts.
-inline int64_t front_words(const BackwardPlan& plan, int64_t n_pos, int heads, int64_t length, int n_buckets) {
+inline int64_t front_words(const BackwardPlan& plan, bool tensor_cores, int64_t n_pos, int heads, int64_t length,
+                           int n_buckets) {
   const int64_t sums = (int64_t)heads * n_buckets;
-  return std::max(plan.dq_words + plan.dkv_words + plan.ctas * sums, n_pos * cdiv(length, TQ) * sums);
+  return tensor_cores ? plan.dq_words + plan.dkv_words + plan.ctas * sums : n_pos * cdiv(length, TQ) * sums;
 }
 
 inline int check(const Args& a, int dtype, const char* what) {
@@ -562,7 +563,9 @@ int mb_bucket_attention_workspace(int dtype, int64_t n_pos, int heads, int kv_he
                  n_buckets > 0,
              "bucket_attention_workspace: bad sizes");
   const bucket::BackwardPlan plan = bucket::backward_plan(n_pos, heads, kv_heads, head_dim, length, dtype);
-  *bytes = 4 * (bucket::front_words(plan, n_pos, heads, length, n_buckets) + n_pos * heads * length);
+  *bytes = 4 * (std::max(bucket::front_words(plan, false, n_pos, heads, length, n_buckets),
+                         bucket::front_words(plan, true, n_pos, heads, length, n_buckets)) +
+                n_pos * heads * length);
   return MB_OK;
 }
 
@@ -595,11 +598,11 @@ int mb_bucket_attention_backward(const void* q, const void* k, const void* v, in
              "bucket_attention_backward: null pointer");
   // one plan for the whole call: the limit on parts may change beside it
   const bucket::BackwardPlan plan = bucket::backward_plan(n_pos, heads, kv_heads, head_dim, length, dtype);
-  const int64_t front = bucket::front_words(plan, n_pos, heads, length, n_buckets);
+  const bool tensor_cores = bucket::tc_serves(a, dtype);
+  const int64_t front = bucket::front_words(plan, tensor_cores, n_pos, heads, length, n_buckets);
   const int64_t need = 4 * (front + n_pos * heads * length);
   MB_REQUIRE(workspace_bytes >= need && aligned(workspace, 16),
              "bucket_attention_backward: the workspace needs %lld bytes, 16-byte aligned", (long long)need);
-  const bool tensor_cores = bucket::tc_serves(a, dtype);
   a.dq_part = (float*)workspace;
   a.dkv_part = a.dq_part + plan.dq_words;
   a.bias_part = tensor_cores ? a.dkv_part + plan.dkv_words : a.dq_part;

@@ -1180,6 +1180,14 @@ def _bucket_workspace(*sizes) -> int:
     return need.value
 
 
+_LARGE_WORKSPACE = 1 << 26  # bytes from which the rows' alignment is worth a look
+
+
+def _rows_on_16(t) -> bool:
+    """The rows that the tensor cores read: bf16 on 16 bytes."""
+    return t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:3])
+
+
 def bucket_attention_limit_parts(limit: int = 0) -> None:
     """Limit the parts of dq that ``bucket_attention_backward`` keeps in its
     workspace to ``limit`` bytes (0: the default, 2 GiB, or four key tiles'
@@ -1207,7 +1215,10 @@ def bucket_attention_backward(q, k, v, bias, bucket_map, coords, valid, out, sta
         raise ValueError("stats.full must be the forward's (P, H, L, d) fp32 tensor")
     grad = grad_out.to(q.dtype)
     grad, o = (t if t.stride(3) == 1 else t.contiguous() for t in (grad, out))
-    need = _bucket_workspace(dtype_code(q.dtype), p, h, k.shape[1], d, length, bias.shape[0])
+    sizes = (p, h, k.shape[1], d, length, bias.shape[0])
+    need = _bucket_workspace(dtype_code(q.dtype), *sizes)
+    if need > _LARGE_WORKSPACE and not all(map(_rows_on_16, (*kept, o, grad))):
+        need = _bucket_workspace(_lib.MB_F32, *sizes)  # the CUDA cores keep no parts of dq, dk and dv
     ws = torch.empty(need, dtype=torch.uint8, device=q.device)
     dq = torch.empty(p, h, length, d, dtype=q.dtype, device=q.device)
     dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)

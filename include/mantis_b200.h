@@ -509,7 +509,8 @@ int mb_bucket_attention(const void* q, const void* k, const void* v, int dtype, 
  * contiguous, in the tensors' type, and dbias (n_buckets, heads) fp32 (NULL
  * skips it). out, full (NULL for fp32) and lse from the forward call; grad_out
  * strided as out may be. Deterministic: no atomics, every sum in a fixed
- * order. workspace: mb_bucket_attention_workspace bytes, 16-byte aligned. */
+ * order. workspace: mb_bucket_attention_workspace bytes, 16-byte aligned; bf16
+ * rows off 16 bytes, which the CUDA cores serve, need no more than f32 ones. */
 int mb_bucket_attention_workspace(int dtype, int64_t n_pos, int heads, int kv_heads, int head_dim, int64_t length,
                                   int n_buckets, int64_t* bytes);
 int mb_bucket_attention_backward(const void* q, const void* k, const void* v, int dtype, int64_t n_pos, int heads,

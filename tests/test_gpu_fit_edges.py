@@ -342,3 +342,29 @@ def test_attention_gradients_within_their_workspace(dtype, d, p, length):
             _within(name, x, y, b)
         assert bool((ws[need:] == 0xA5).all())
     mb._lib.check_device_error()
+
+
+def test_attention_gradients_of_unaligned_rows_reserve_no_parts():
+    """bf16 rows off 16 bytes run on the CUDA cores: beside the gradients they
+    need delta and the bias sums (4 MiB here), not the 1 GiB of dQ's parts that
+    the same rows on 16 bytes keep, and the results agree."""
+    p, h, length, d = 64, 8, 1024, 64
+    g = torch.Generator(device=DEV).manual_seed(1)
+    rows = [torch.randn(p, h, length, d + 1, generator=g, device=DEV).bfloat16() for _ in range(3)]
+    bmap = torch.from_numpy(mb.hexgraph.line_buckets()).to(DEV)
+    bias = torch.randn(32, h, generator=g, device=DEV)
+    t = torch.arange(length, dtype=torch.int32, device=DEV)
+    where = bias, bmap, torch.stack([t, torch.zeros_like(t)], -1).contiguous(), None
+    results, extra = [], []
+    for q, k, v in ([r[..., 1:] for r in rows], [r[..., 1:].contiguous() for r in rows]):
+        out, st = ops.bucket_attention(q, k, v, *where, for_backward=True)
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        grads = ops.bucket_attention_backward(q, k, v, *where, out, st, out)
+        extra.append(torch.cuda.max_memory_allocated() - before - sum(x.numel() * x.element_size() for x in grads))
+        results.append(grads)
+    assert extra[0] <= 8 << 20 and extra[1] >= 1 << 30
+    # P and dS are rounded to bf16 on the tensor cores alone: 2^-9 of terms, 2^-7 of the largest sum
+    for x, y in zip(*results):
+        assert float((x.float() - y.float()).abs().max()) <= 2.0 ** -7 * float(y.float().abs().max())
+    mb._lib.check_device_error()
